@@ -34,7 +34,7 @@ __global__ __launch_bounds__(NT, LOW == 1 ? 6 : 4) void plane_kernel(const ScanA
 {
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     constexpr int WPP = NT / 64;                                        // all waves: one team on the plane-row
-    static_assert(CPT % 4 == 0, "columns are stepped four at a time");
+    static_assert(CPT % 4 == 0 && CPT <= 64, "columns are stepped four at a time; lane l keeps the ballot of column l");
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     // workgroup -> (sub-block, plane).  Workgroup ids go round-robin over the 8 XCDs; k = the index within the XCD.  Plane 0
@@ -162,7 +162,20 @@ __global__ __launch_bounds__(NT, LOW == 1 ? 6 : 4) void plane_kernel(const ScanA
     }
     const int emit_from = __builtin_amdgcn_readfirstlane(a.row0 > blk_beg ? (int)(a.row0 - blk_beg) : 0);   // first relative row whose ballots leave
 
-    uint64_t *hnext = hout + ((int64_t)blk_beg - a.h_row0) * a.n_chunks + chunk0;   // this wave's ballots of the row to be walked next
+    // The ballots of a row: lane l of the wave keeps the one of column l (two v_writelane per column: one scalar operand and a
+    // constant lane, no lane mask to hold), and ONE vector store of up to 8 * CPT consecutive bytes takes them out.  It is
+    // issued at the top of the NEXT row, beside that row's prefetch: the compiler waits for every outstanding memory operation
+    // behind the walk and at the end of the loop (its loads sit behind branches), so a store anywhere else is waited for at once.
+    // Bound by VALU issue and the row's chain of phases, not by these bytes (2.5 GB of 12 ms): 100,000 samples x 1,000,000 sites,
+    // every 20th: 12.5 ms (80.2 M sites/s); 32,488 x 142,000, every 13th: 0.93 ms; 50,000 x 1,000,000, every 10th: 8.7 ms.
+    uint64_t *hput = hout + ((int64_t)blk_beg + emit_from - a.h_row0) * a.n_chunks + chunk0;   // this wave's part of the next row to leave
+    const int n_mine = a.n_chunks - chunk0 < CPT ? a.n_chunks - chunk0 : CPT;                 // its columns that exist (none: <= 0)
+    uint32_t keep_lo = 0, keep_hi = 0;
+    auto put_ballots = [&](int i) {                                      // i: the relative row that keep_lo / keep_hi hold
+        if (i < emit_from) return;                                       // wave-uniform
+        if (lane < n_mine) hput[lane] = (uint64_t)keep_hi << 32 | keep_lo;
+        hput += a.n_chunks;                                              // (a running pointer: no 64-bit multiply per row on the scalar unit)
+    };
     // (profiling build only: cycles per phase -- 0 walk, 1 toggles, 2 barrier, 3 directory, 4 barrier)
     unsigned long long tsum[8] = {0, 0, 0, 0, 0, 0, 0, 0}, tlast = BGTH_TIMES(a) ? __builtin_amdgcn_s_memtime() : 0ull;
     // Loop (iteration -1 only prepares row blk_beg):   walk(row) + toggles(row+1) | directory(row+1) |     two barriers per row
@@ -172,21 +185,11 @@ __global__ __launch_bounds__(NT, LOW == 1 ? 6 : 4) void plane_kernel(const ScanA
         const uint64_t d_ahead = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(d_next >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)d_next);
         const Ahead ahead = load_ahead(i + 2, d_ahead);
         d_next = load_desc(i + 3);
+        put_ballots(i - 1);
         if (walking && !(BGTH_SKIP(a, 0x10000))) {                       // (profiling build: 0x10000 no walk, 0x20000 no toggles,
             const uint32_t base = lds0 - 8u;                             //  0x40000 no directory trips, 0x80000 no barriers -- timing only)
             const uint32_t n0 = 0u - n0s[i & 1];
-            // chunks of this wave whose ballots leave in this row, as ONE scalar integer: as a boolean per column the test was kept
-            // in 64-bit lane masks, spilled to VGPR lanes and read back with two v_readlane per column and row
-            const int n_emit = __builtin_amdgcn_readfirstlane(i >= emit_from ? a.n_chunks - chunk0 : 0);
             [[maybe_unused]] uint32_t ca = 0, cb = 0, cc = 0;
-            // The ballots leave straight from their SGPRs: one scalar store per column (s_store_dwordx2, written back by the
-            // s_dcache_wb at the end of the kernel) instead of moving them into lanes first (two v_cndmask per column: a
-            // quarter of this walk's VALU instructions).
-            // A scalar store reads its data registers when it EXECUTES, not when it issues: the ballots of a group stay in
-            // their SGPRs (pm) until the next statement's opening s_waitcnt lgkmcnt(0) has retired the stores.
-            uint64_t *hrow = hnext;                                      // (a running pointer: no 64-bit multiply per row on the scalar unit)
-            hnext += a.n_chunks;
-            uint64_t pm[4] = {0, 0, 0, 0};
 #pragma unroll
             for (int j = 0; j < CPT; j += 4) {
                 // a wave's priority falls as it gets through its columns (2 -> 1 -> 0 at 40 % and 80 %), so that the waves of a
@@ -203,16 +206,19 @@ __global__ __launch_bounds__(NT, LOW == 1 ? 6 : 4) void plane_kernel(const ScanA
                 uint64_t m0[4] = {0, 0, 0, 0}, m1[4] = {0, 0, 0, 0};
                 if constexpr (LOW == 1) step4_plane_low(q0, m0, base, n0);
                 else step4<true>(q0, q1, m0, m1, ca, cb, cc, base, 0u, n0, 0u);
-                asm volatile("" :: "s"(pm[0]), "s"(pm[1]), "s"(pm[2]), "s"(pm[3]));
 #pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    rk_[j + u] = q0[u];
-                    if (j + u < n_emit)                                    // wave-uniform
-                        asm volatile("s_store_dwordx2 %0, %1, %2" :: "s"(m0[u]), "s"(hrow), "n"((j + u) * 8) : "memory");
-                    pm[u] = m0[u];
-                }
+                for (int u = 0; u < 4; ++u) rk_[j + u] = q0[u];
+                // (one statement, the oldest ballot first: nine VALU instructions lie between the row step's last v_cmp and the
+                // v_writelane that reads its SGPRs -- the compiler, which does not look into the row step, need not space them)
+                asm("v_writelane_b32 %0, %2, %10\n\tv_writelane_b32 %1, %3, %10\n\t"
+                    "v_writelane_b32 %0, %4, %11\n\tv_writelane_b32 %1, %5, %11\n\t"
+                    "v_writelane_b32 %0, %6, %12\n\tv_writelane_b32 %1, %7, %12\n\t"
+                    "v_writelane_b32 %0, %8, %13\n\tv_writelane_b32 %1, %9, %13"
+                    : "+v"(keep_lo), "+v"(keep_hi)
+                    : "s"((uint32_t)m0[0]), "s"((uint32_t)(m0[0] >> 32)), "s"((uint32_t)m0[1]), "s"((uint32_t)(m0[1] >> 32)),
+                      "s"((uint32_t)m0[2]), "s"((uint32_t)(m0[2] >> 32)), "s"((uint32_t)m0[3]), "s"((uint32_t)(m0[3] >> 32)),
+                      "n"(j), "n"(j + 1), "n"(j + 2), "n"(j + 3));
             }
-            asm volatile("s_waitcnt lgkmcnt(0)" :: "s"(pm[0]), "s"(pm[1]), "s"(pm[2]), "s"(pm[3]) : "memory");
         }
         BGTH_TICK(0);
         // The build of the next row is a latency chain of few instructions (decode, LDS atomics, prefix scans, two barriers):
@@ -232,7 +238,7 @@ __global__ __launch_bounds__(NT, LOW == 1 ? 6 : 4) void plane_kernel(const ScanA
         if (BGTH_WALK_PRIO(a)) __builtin_amdgcn_s_setprio(0);
         BGTH_TICK(4);
     }
-    asm volatile("s_dcache_wb\n\ts_waitcnt lgkmcnt(0)" ::: "memory");     // the scalar stores of the ballots reach memory
+    put_ballots(nrows - 1);
 #ifdef BGTH_ABLATE
     if (BGTH_TIMES(a) && lane == 0) for (int i = 0; i < 8; ++i) atomicAdd(a.debug_times + i, tsum[i]);
 #endif
