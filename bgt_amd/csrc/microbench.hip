@@ -190,13 +190,12 @@ __device__ __forceinline__ void op_block()
     if constexpr (OP == 42) asm volatile("v_and_b32 v40, 0xffffffe0, v40\n\tv_and_b32 v41, 0xffffffe0, v41\n\tv_and_b32 v42, 0xffffffe0, v42\n\tv_and_b32 v43, 0xffffffe0, v43\n\tv_and_b32 v44, 0xffffffe0, v44\n\tv_and_b32 v45, 0xffffffe0, v45\n\tv_and_b32 v46, 0xffffffe0, v46\n\tv_and_b32 v47, 0xffffffe0, v47\n\t" ::: "v40","v41","v42","v43","v44","v45","v46","v47","v48","v49","v50","v51","v52","v53","v54","v55","v56","v57","v58","v59","vcc","s20","s21","s22","s23","s24");
     if constexpr (OP == 43) asm volatile("v_add_u32 v40, v48, v40\n\tv_add_u32 v41, v48, v41\n\tv_add_u32 v42, v48, v42\n\tv_add_u32 v43, v48, v43\n\tv_add_u32 v44, v48, v44\n\tv_add_u32 v45, v48, v45\n\tv_add_u32 v46, v48, v46\n\tv_add_u32 v47, v48, v47\n\t" ::: "v40","v41","v42","v43","v44","v45","v46","v47","v48","v49","v50","v51","v52","v53","v54","v55","v56","v57","v58","v59","vcc","s20","s21","s22","s23","s24");
     if constexpr (OP == 44) asm volatile("v_fma_f32 v40, v40, v48, v49\n\tv_fma_f32 v41, v41, v48, v49\n\tv_fma_f32 v42, v42, v48, v49\n\tv_fma_f32 v43, v43, v48, v49\n\tv_fma_f32 v44, v44, v48, v49\n\tv_fma_f32 v45, v45, v48, v49\n\tv_fma_f32 v46, v46, v48, v49\n\tv_fma_f32 v47, v47, v48, v49\n\t" ::: "v40","v41","v42","v43","v44","v45","v46","v47","v48","v49","v50","v51","v52","v53","v54","v55","v56","v57","v58","v59","vcc","s20","s21","s22","s23","s24");
-    if constexpr (OP == 45) asm volatile("v_pk_fma_f32 v[40:41], v[40:41], v[56:57], v[58:59]\n\tv_pk_fma_f32 v[42:43], v[42:43], v[56:57], v[58:59]\n\tv_pk_fma_f32 v[44:45], v[44:45], v[56:57], v[58:59]\n\tv_pk_fma_f32 v[46:47], v[46:47], v[56:57], v[58:59]\n\tv_pk_fma_f32 v[56:57], v[56:57], v[56:57], v[58:59]\n\tv_pk_fma_f32 v[58:59], v[58:59], v[56:57], v[58:59]\n\tv_pk_fma_f32 v[52:53], v[52:53], v[56:57], v[58:59]\n\tv_pk_fma_f32 v[54:55], v[54:55], v[56:57], v[58:59]\n\t" ::: "v40","v41","v42","v43","v44","v45","v46","v47","v48","v49","v50","v51","v52","v53","v54","v55","v56","v57","v58","v59","vcc","s20","s21","s22","s23","s24");
-    if constexpr (OP == 46) asm volatile("v_lshlrev_b64 v[40:41], 3, v[40:41]\n\tv_lshlrev_b64 v[42:43], 3, v[42:43]\n\tv_lshlrev_b64 v[44:45], 3, v[44:45]\n\tv_lshlrev_b64 v[46:47], 3, v[46:47]\n\tv_lshlrev_b64 v[56:57], 3, v[56:57]\n\tv_lshlrev_b64 v[58:59], 3, v[58:59]\n\tv_lshlrev_b64 v[52:53], 3, v[52:53]\n\tv_lshlrev_b64 v[54:55], 3, v[54:55]\n\t" ::: "v40","v41","v42","v43","v44","v45","v46","v47","v48","v49","v50","v51","v52","v53","v54","v55","v56","v57","v58","v59","vcc","s20","s21","s22","s23","s24");
-    if constexpr (OP == 47) asm volatile("v_readlane_b32 s24, v40, 3\n\tv_readlane_b32 s24, v41, 3\n\tv_readlane_b32 s24, v42, 3\n\tv_readlane_b32 s24, v43, 3\n\tv_readlane_b32 s24, v44, 3\n\tv_readlane_b32 s24, v45, 3\n\tv_readlane_b32 s24, v46, 3\n\tv_readlane_b32 s24, v47, 3\n\t" ::: "v40","v41","v42","v43","v44","v45","v46","v47","v48","v49","v50","v51","v52","v53","v54","v55","v56","v57","v58","v59","vcc","s20","s21","s22","s23","s24");
-    if constexpr (OP == 48) asm volatile("v_mad_u64_u32 v[40:41], vcc, v40, v56, v[40:41]\n\tv_mad_u64_u32 v[42:43], vcc, v42, v56, v[42:43]\n\tv_mad_u64_u32 v[44:45], vcc, v44, v56, v[44:45]\n\tv_mad_u64_u32 v[46:47], vcc, v46, v56, v[46:47]\n\tv_mad_u64_u32 v[56:57], vcc, v56, v56, v[56:57]\n\tv_mad_u64_u32 v[58:59], vcc, v50, v56, v[58:59]\n\tv_mad_u64_u32 v[52:53], vcc, v52, v56, v[52:53]\n\tv_mad_u64_u32 v[54:55], vcc, v54, v56, v[54:55]\n\t" ::: "v40","v41","v42","v43","v44","v45","v46","v47","v48","v49","v50","v51","v52","v53","v54","v55","v56","v57","v58","v59","vcc","s20","s21","s22","s23","s24");
+    if constexpr (OP == 45) asm volatile("v_lshlrev_b64 v[40:41], 3, v[40:41]\n\tv_lshlrev_b64 v[42:43], 3, v[42:43]\n\tv_lshlrev_b64 v[44:45], 3, v[44:45]\n\tv_lshlrev_b64 v[46:47], 3, v[46:47]\n\tv_lshlrev_b64 v[56:57], 3, v[56:57]\n\tv_lshlrev_b64 v[58:59], 3, v[58:59]\n\tv_lshlrev_b64 v[52:53], 3, v[52:53]\n\tv_lshlrev_b64 v[54:55], 3, v[54:55]\n\t" ::: "v40","v41","v42","v43","v44","v45","v46","v47","v48","v49","v50","v51","v52","v53","v54","v55","v56","v57","v58","v59","vcc","s20","s21","s22","s23","s24");
+    if constexpr (OP == 46) asm volatile("v_readlane_b32 s24, v40, 3\n\tv_readlane_b32 s24, v41, 3\n\tv_readlane_b32 s24, v42, 3\n\tv_readlane_b32 s24, v43, 3\n\tv_readlane_b32 s24, v44, 3\n\tv_readlane_b32 s24, v45, 3\n\tv_readlane_b32 s24, v46, 3\n\tv_readlane_b32 s24, v47, 3\n\t" ::: "v40","v41","v42","v43","v44","v45","v46","v47","v48","v49","v50","v51","v52","v53","v54","v55","v56","v57","v58","v59","vcc","s20","s21","s22","s23","s24");
+    if constexpr (OP == 47) asm volatile("v_mad_u64_u32 v[40:41], vcc, v40, v56, v[40:41]\n\tv_mad_u64_u32 v[42:43], vcc, v42, v56, v[42:43]\n\tv_mad_u64_u32 v[44:45], vcc, v44, v56, v[44:45]\n\tv_mad_u64_u32 v[46:47], vcc, v46, v56, v[46:47]\n\tv_mad_u64_u32 v[56:57], vcc, v56, v56, v[56:57]\n\tv_mad_u64_u32 v[58:59], vcc, v50, v56, v[58:59]\n\tv_mad_u64_u32 v[52:53], vcc, v52, v56, v[52:53]\n\tv_mad_u64_u32 v[54:55], vcc, v54, v56, v[54:55]\n\t" ::: "v40","v41","v42","v43","v44","v45","v46","v47","v48","v49","v50","v51","v52","v53","v54","v55","v56","v57","v58","v59","vcc","s20","s21","s22","s23","s24");
 }
-static const char *const kOpName[] = {"v_mov_b32", "v_and_b32", "v_or_b32", "v_xor_b32", "v_sub_u32", "v_lshrrev_b32 imm", "v_ashrrev_i32 imm", "v_lshlrev_b32 imm", "v_lshlrev_b32 vgpr", "v_lshl_add_u32", "v_add_lshl_u32", "v_and_or_b32", "v_lshl_or_b32", "v_or3_b32", "v_add3_u32", "v_bfe_u32", "v_bfe_i32", "v_bfi_b32", "v_alignbit_b32", "v_perm_b32", "v_bitop3_b32", "v_cndmask_b32 vcc", "v_cndmask_b32_e64 sgpr", "v_cmp_gt_i32 vcc", "v_cmp_gt_i32_e64 sgpr", "v_mul_u32_u24", "v_mad_u32_u24", "v_mad_i32_i24", "v_mul_lo_u32", "v_mul_hi_u32", "v_min_u32", "v_mbcnt_lo_u32_b32", "v_ffbh_u32", "v_bcnt_u32_b32", "v_add_co_u32", "v_xad_u32", "v_sad_u32", "v_add_u32 dpp row_shr", "v_mov_b32 dpp row_shr", "v_pk_add_u16", "v_cvt_f32_u32", "v_subrev_u32 sgpr", "v_and_b32 literal", "v_add_u32", "v_fma_f32", "v_pk_fma_f32", "v_lshlrev_b64", "v_readlane_b32", "v_mad_u64_u32"};
-constexpr int kNumOps = 49;
+static const char *const kOpName[] = {"v_mov_b32", "v_and_b32", "v_or_b32", "v_xor_b32", "v_sub_u32", "v_lshrrev_b32 imm", "v_ashrrev_i32 imm", "v_lshlrev_b32 imm", "v_lshlrev_b32 vgpr", "v_lshl_add_u32", "v_add_lshl_u32", "v_and_or_b32", "v_lshl_or_b32", "v_or3_b32", "v_add3_u32", "v_bfe_u32", "v_bfe_i32", "v_bfi_b32", "v_alignbit_b32", "v_perm_b32", "v_bitop3_b32", "v_cndmask_b32 vcc", "v_cndmask_b32_e64 sgpr", "v_cmp_gt_i32 vcc", "v_cmp_gt_i32_e64 sgpr", "v_mul_u32_u24", "v_mad_u32_u24", "v_mad_i32_i24", "v_mul_lo_u32", "v_mul_hi_u32", "v_min_u32", "v_mbcnt_lo_u32_b32", "v_ffbh_u32", "v_bcnt_u32_b32", "v_add_co_u32", "v_xad_u32", "v_sad_u32", "v_add_u32 dpp row_shr", "v_mov_b32 dpp row_shr", "v_pk_add_u16", "v_cvt_f32_u32", "v_subrev_u32 sgpr", "v_and_b32 literal", "v_add_u32", "v_fma_f32", "v_lshlrev_b64", "v_readlane_b32", "v_mad_u64_u32"};
+constexpr int kNumOps = sizeof(kOpName) / sizeof(kOpName[0]);
 
 template <int OP>
 __global__ void op_rate_kernel(int iters, unsigned long long *cycles, uint32_t *sink)

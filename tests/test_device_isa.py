@@ -61,3 +61,10 @@ def test_no_write_through_the_scalar_data_cache(mnemonics):
     scalar = {n for n in mnemonics if n.startswith("s_")}
     bad = sorted(n for n in scalar if "store" in n or "atomic" in n or ("cache" in n and not n.endswith(("_inv", "_inv_vol"))))
     assert not bad, bad
+
+
+def test_no_packed_fp32_arithmetic(mnemonics):
+    """The device code is built without the packed-FP32 feature (bgt_amd/csrc/Makefile): neither written by hand, which the assembler
+    then refuses, nor made by the compiler out of ordinary float code."""
+    bad = sorted(n for n in mnemonics if n.startswith("v_pk_") and n.split("_e")[0].endswith("_f32"))
+    assert not bad, bad
