@@ -166,8 +166,8 @@ __global__ __launch_bounds__(NT, LOW == 1 ? 6 : 4) void plane_kernel(const ScanA
     // constant lane, no lane mask to hold), and ONE vector store of up to 8 * CPT consecutive bytes takes them out.  It is
     // issued at the top of the NEXT row, beside that row's prefetch: the compiler waits for every outstanding memory operation
     // behind the walk and at the end of the loop (its loads sit behind branches), so a store anywhere else is waited for at once.
-    // Bound by VALU issue and the row's chain of phases, not by these bytes (2.5 GB of 12 ms): 100,000 samples x 1,000,000 sites,
-    // every 20th: 12.5 ms (80.2 M sites/s); 32,488 x 142,000, every 13th: 0.93 ms; 50,000 x 1,000,000, every 10th: 8.7 ms.
+    // The kernel is bound by VALU issue and the row's chain of phases, not by these bytes (2.5 GB in 12 ms).  rocprofv3, 25 launches:
+    // 100,000 samples x 1,000,000 sites, every 20th: 12.03 ms; 32,488 x 142,000, every 13th: 0.864 ms.
     uint64_t *hput = hout + ((int64_t)blk_beg + emit_from - a.h_row0) * a.n_chunks + chunk0;   // this wave's part of the next row to leave
     const int n_mine = a.n_chunks - chunk0 < CPT ? a.n_chunks - chunk0 : CPT;                 // its columns that exist (none: <= 0)
     uint32_t keep_lo = 0, keep_hi = 0;
